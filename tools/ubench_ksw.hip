@@ -4,12 +4,10 @@
 // cell, four traceback compares, H update, the two threshold compares) `iters` times per wave at 8 waves per SIMD and
 // reports wall-clock nanoseconds per (alignment, diagonal).  The values are synthetic; only the instruction stream matters.
 //   V0  one alignment per wave, int8 in the top byte, compare -> v_addc traceback (the round-3 kernel)
-//   V1  same, the four compare masks leave by two s_store_dwordx4 per diagonal
 //   V2  two alignments per wave in 16-bit halves (v_pk_*), SDWA compares -> v_addc, 32-bit H per alignment
-//   V3  as V2, masks leave by four s_store_dwordx4
 //   V4  as V2 with H kept as a packed 16-bit offset
-//   V5  as V3 with H kept as a packed 16-bit offset
 //   V6  packed, traceback bits gathered from saturating differences (no compares), packed H
+// The traceback leaves every variant by ordinary vector stores.  (V1, V3 and V5 no longer exist.)
 // Also the issue rate of the few ops the earlier table lacks.
 //   hipcc --offload-arch=gfx950 -O3 -o gpurun_out/ubench_ksw tools/ubench_ksw.hip && gpurun_out/ubench_ksw
 #include <hip/hip_runtime.h>
@@ -18,8 +16,6 @@
 #include <vector>
 
 #define CHECK(x) do { hipError_t e_ = (x); if (e_ != hipSuccess) { fprintf(stderr, "%s: %s\n", #x, hipGetErrorString(e_)); exit(1); } } while (0)
-
-typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ int lane_id() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
 __device__ __forceinline__ int dppz_shr1(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x138, 0xf, 0xf, true); }
@@ -47,12 +43,6 @@ __device__ __forceinline__ unsigned long long cmp_gt_hi(unsigned a, unsigned b) 
 __device__ __forceinline__ unsigned long long cmp_ne0_lo(unsigned a) { unsigned long long m; asm("v_cmp_ne_u16_sdwa %0, %1, %2 src0_sel:WORD_0 src1_sel:DWORD" : "=s"(m) : "v"(a), "v"(0)); return m; }
 __device__ __forceinline__ unsigned long long cmp_ne0_hi(unsigned a) { unsigned long long m; asm("v_cmp_ne_u16_sdwa %0, %1, %2 src0_sel:WORD_1 src1_sel:DWORD" : "=s"(m) : "v"(a), "v"(0)); return m; }
 
-__device__ __forceinline__ void sstore4(unsigned long long m0, unsigned long long m1, unsigned long long base, unsigned off)
-{
-	u4 d = {(unsigned)m0, (unsigned)(m0 >> 32), (unsigned)m1, (unsigned)(m1 >> 32)};
-	asm volatile("s_store_dwordx4 %0, %1, %2" :: "s"(d), "s"(base), "s"(off) : "memory");
-}
-
 struct Res { long long cycles; };
 
 template <int V>
@@ -64,9 +54,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(8))) void k
 	for (int i = threadIdx.x; i < 2048 + 64; i += blockDim.x) lds[i] = (unsigned)(((i * 2654435761u) >> 13) & 3) + 1 << 24 | 0x000c0c0cu | (((i * 40503u) >> 7) & 3) + 1 << 8;
 	__syncthreads();
 	unsigned *row = gbuf + (size_t)wave * (wave_bytes / 4);
-	const unsigned long long sbase = (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned long long)row)) |
-	                                 ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned long long)row >> 32)) << 32);
-	unsigned soff = 0;
 	const unsigned *qptr = lds + 2048 + lane;
 	int XA = 0, VA = lane << 20, UA = 0, YA = 0, ZA = 10 << 24, HA = -lane, HA1 = -lane * 2;
 	unsigned T0 = 0x0b080808u + lane, T1 = 0x080b0808u;
@@ -78,7 +65,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(8))) void k
 	const long long t0 = clock64();
 	for (int r = 0; r < iters; ++r) {
 		const unsigned sel = *qptr; qptr -= 1;
-		if (V <= 1) {
+		if (V == 0) {
 			const int xp = dppz_shr1(XA), vp = dppz_shr1(VA), Hp = dppz_shr1(HA);
 			const int zn = (int)__builtin_amdgcn_perm(T0, T1, sel);
 			ZA = lane_in(geLoM) ? zn : ZA;
@@ -93,12 +80,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(8))) void k
 			const int a2 = a - zq, b2 = b - zq;
 			const unsigned long long c3 = ballot(a2 > 0), c4 = ballot(b2 > 0);
 			XA = a2 > 0 ? a2 : 0; YA = b2 > 0 ? b2 : 0; UA = un; VA = vn;
-			if (V == 0) {
-				accA = shl1_in(accA, c1); accA = shl1_in(accA, c2); accA = shl1_in(accA, c3); accA = shl1_in(accA, c4);
-				if ((r & 7) == 7) row[(r >> 3) * 64 + lane] = accA;
-			} else {
-				sstore4(c1, c2, sbase, soff); sstore4(c3, c4, sbase, soff + 16); soff += 32;
-			}
+			accA = shl1_in(accA, c1); accA = shl1_in(accA, c2); accA = shl1_in(accA, c3); accA = shl1_in(accA, c4);
+			if ((r & 7) == 7) row[(r >> 3) * 64 + lane] = accA;
 			const bool sp = lane_in(spM);
 			const int h = (sp ? Hp : HA) + (int)((unsigned)(sp ? un : vn) >> 24);
 			HA = lane_in(geLoM) ? h : HA;
@@ -133,19 +116,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(8))) void k
 				const unsigned long long c2l = cmp_gt_lo(b, zz1), c2h = cmp_gt_hi(b, zz1);
 				const unsigned long long c3l = cmp_ne0_lo(xn), c3h = cmp_ne0_hi(xn);
 				const unsigned long long c4l = cmp_ne0_lo(yn), c4h = cmp_ne0_hi(yn);
-				if (V == 2 || V == 4) {
-					accA = shl1_in(accA, c1l); accA = shl1_in(accA, c2l); accA = shl1_in(accA, c3l); accA = shl1_in(accA, c4l);
-					accB = shl1_in(accB, c1h); accB = shl1_in(accB, c2h); accB = shl1_in(accB, c3h); accB = shl1_in(accB, c4h);
-					if ((r & 7) == 7) { row[(r >> 3) * 128 + lane] = accA; row[(r >> 3) * 128 + 64 + lane] = accB; }
-				} else {
-					sstore4(c1l, c2l, sbase, soff); sstore4(c3l, c4l, sbase, soff + 16);
-					sstore4(c1h, c2h, sbase, soff + 32); sstore4(c3h, c4h, sbase, soff + 48); soff += 64;
-				}
+				accA = shl1_in(accA, c1l); accA = shl1_in(accA, c2l); accA = shl1_in(accA, c3l); accA = shl1_in(accA, c4l);
+				accB = shl1_in(accB, c1h); accB = shl1_in(accB, c2h); accB = shl1_in(accB, c3h); accB = shl1_in(accB, c4h);
+				if ((r & 7) == 7) { row[(r >> 3) * 128 + lane] = accA; row[(r >> 3) * 128 + 64 + lane] = accB; }
 			}
 			XA = (int)xn; YA = (int)yn; UA = (int)un; VA = (int)vn;
 			const bool sp = lane_in(spM);
 			const unsigned uv = sp ? un : vn;
-			if (V == 2 || V == 3) {
+			if (V == 2) {
 				const int Hp0 = dppz_shr1(HA), Hp1 = dppz_shr1(HA1);
 				const int h0 = (sp ? Hp0 : HA) + (int)((uv >> 8) & 0xffu);
 				const int h1 = (sp ? Hp1 : HA1) + (int)(uv >> 24);
@@ -179,10 +157,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(8))) void k
 			}
 		}
 		if (r & 1) geLoM = (geLoM << 1) | (geLoM >> 63); else spM = (spM << 1) | (spM >> 63);
-		if ((r & 31) == 31) { qptr += 32; soff = 0; }
+		if ((r & 31) == 31) qptr += 32;
 		if ((r & 1023) == 1023) qptr = lds + 2048 + lane;
 	}
-	if (V == 1 || V == 3 || V == 5) asm volatile("s_dcache_wb\n s_waitcnt lgkmcnt(0)" ::: "memory");
 	const long long t1 = clock64();
 	if (lane == 0) out[wave].cycles = t1 - t0;
 	if (XA + VA + UA + YA + ZA + HA + HA1 + (int)accA + (int)accB + thrI + thrI1 == 0x7fffffff) *sink = 1;
@@ -264,56 +241,6 @@ __global__ void k_op(Res *out, int iters, int *sink)
 	if (v0 + v1 + v2 + v3 + v4 + v5 + v6 + v7 + s0 == 0x7fffffff) *sink = 1;
 }
 
-
-// ---- are scalar stores safe when the data SGPRs are overwritten right behind them?  every iteration writes two fresh compare
-// masks into the SAME four SGPRs and stores them with no wait; the host recomputes every mask ----
-__global__ __launch_bounds__(512) void k_sstore_check(unsigned *gbuf, size_t wave_bytes, int iters)
-{
-	const int lane = lane_id();
-	const int wave = (int)(blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6));
-	unsigned *row = gbuf + (size_t)wave * (wave_bytes / 4);
-	const unsigned long long sbase = (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned long long)row)) |
-	                                 ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned long long)row >> 32)) << 32);
-	unsigned soff = 0;
-	for (int r = 0; r < iters; ++r) {
-		const unsigned x = ((unsigned)lane * 2654435761u + (unsigned)r * 40503u + (unsigned)wave * 977u) >> 7;
-		const unsigned y = ((unsigned)lane * 40503u + (unsigned)r * 2654435761u) >> 7;
-		asm volatile("v_cmp_gt_u32_e64 s[20:21], %0, %1\n v_cmp_lt_u32_e64 s[22:23], %0, %2\n s_nop 1\n s_store_dwordx4 s[20:23], %3, %4"
-		             :: "v"(x), "v"(y), "v"(y ^ 0x5555u), "s"(sbase), "s"(soff) : "s20", "s21", "s22", "s23", "memory");
-		soff += 16;
-	}
-	asm volatile("s_dcache_wb\n s_waitcnt lgkmcnt(0)" ::: "memory");
-}
-
-static void run_check(int cus)
-{
-	const int iters = 2048, W = 8;
-	const size_t wave_bytes = (size_t)iters * 16;
-	const size_t nw = (size_t)cus * 4 * W;
-	unsigned *gbuf;
-	CHECK(hipMalloc(&gbuf, nw * wave_bytes));
-	CHECK(hipMemset(gbuf, 0xee, nw * wave_bytes));
-	hipLaunchKernelGGL(k_sstore_check, dim3(cus * 4), dim3(64 * W), 0, 0, gbuf, wave_bytes, iters);
-	CHECK(hipDeviceSynchronize());
-	std::vector<unsigned> h(nw * wave_bytes / 4);
-	CHECK(hipMemcpy(h.data(), gbuf, nw * wave_bytes, hipMemcpyDeviceToHost));
-	size_t bad = 0, first = (size_t)-1;
-	for (size_t w = 0; w < nw; ++w)
-		for (int r = 0; r < iters; ++r) {
-			unsigned long long m0 = 0, m1 = 0;
-			for (int lane = 0; lane < 64; ++lane) {
-				const unsigned x = ((unsigned)lane * 2654435761u + (unsigned)r * 40503u + (unsigned)w * 977u) >> 7;
-				const unsigned y = ((unsigned)lane * 40503u + (unsigned)r * 2654435761u) >> 7;
-				if (x > y) m0 |= 1ull << lane;
-				if (x < (y ^ 0x5555u)) m1 |= 1ull << lane;
-			}
-			const unsigned *p = &h[(w * iters + r) * 4];
-			if (p[0] != (unsigned)m0 || p[1] != (unsigned)(m0 >> 32) || p[2] != (unsigned)m1 || p[3] != (unsigned)(m1 >> 32)) { if (!bad) first = w * iters + r; ++bad; }
-		}
-	printf("scalar-store check: %zu waves x %d stores of 16 bytes, %zu wrong (first at %zd)\n", nw, iters, bad, (ssize_t)first);
-	CHECK(hipFree(gbuf));
-}
-
 static int g_khz = 2400000;
 
 template <int V>
@@ -378,13 +305,9 @@ int main()
 	const int cus = pr.multiProcessorCount;
 	g_khz = pr.clockRate;
 	printf("%s, %d CUs, clock %d kHz\n", pr.gcnArchName, cus, pr.clockRate);
-	run_check(cus);
 	run_step<0>("V0 single, top byte, addc traceback", cus, 1);
-	run_step<1>("V1 single, top byte, s_store traceback", cus, 1);
 	run_step<2>("V2 pair pk16, sdwa cmp + addc, H 32-bit", cus, 2);
-	run_step<3>("V3 pair pk16, sdwa cmp + s_store, H 32-bit", cus, 2);
 	run_step<4>("V4 pair pk16, sdwa cmp + addc, H packed", cus, 2);
-	run_step<5>("V5 pair pk16, sdwa cmp + s_store, H packed", cus, 2);
 	run_step<6>("V6 pair pk16, sign-gather traceback, H packed", cus, 2);
 	run_op<0>("v_cndmask_b32 sgpr mask", cus);
 	run_op<1>("v_cmp_gt_i16_sdwa", cus);
