@@ -8,6 +8,7 @@
 #   run on this one GPU (1.25 M regions in 8 resident chunks), the issue-rate microbenchmark.
 cd "$(dirname "$0")/.." || exit 1
 export TMPDIR=/tmp
+python3 tools/ubench.py check || exit 1      # (built on the build host: tools/ubench.py build)
 OUT=gpurun_out/prof
 rm -rf $OUT; mkdir -p $OUT
 ARGS="--steps 5 --warmup 2 --no-cpu --no-e2e --no-check --no-other"
@@ -28,7 +29,7 @@ stats c5 --config C5 --steps 5 --warmup 2 --no-cpu --no-e2e --no-check
 # round 6: the regions of 257-600 reads (wide combine build): the byte-based k_assemble passes must stay empty
 stats deep --config deep --regions 10000 --steps 3 --warmup 2 --in-flight 1 --sub-batches 2 --no-cpu --no-e2e --no-check
 python3 bench.py --config deep --regions 10000 --steps 3 --warmup 2 --in-flight 1 --sub-batches 2 --no-cpu --no-e2e > $OUT/deep_bench.json 2>> $OUT/err
-timeout 120 tools/ubench_wany.bin > $OUT/ubench_wany.txt 2>&1
+python3 tools/ubench.py run wany $OUT/ubench_wany.txt || exit 1
 : > $OUT/other_workloads.jsonl
 python3 bench.py --config C3 --steps 3 --warmup 1 --no-cpu --no-e2e >> $OUT/other_workloads.jsonl 2>> $OUT/err
 python3 bench.py --config C5 --no-cpu --no-e2e >> $OUT/other_workloads.jsonl 2>> $OUT/err
@@ -39,8 +40,8 @@ python3 bench.py --no-cpu --no-e2e --no-check --no-other --in-flight 1 --lockste
 python3 bench.py --knob asm_v1=1 --no-cpu --no-e2e --no-check --no-other >> $OUT/other_workloads.jsonl 2>> $OUT/err
 python3 bench.py --config C3 --knob no_rich=1 --steps 3 --warmup 1 --no-cpu --no-e2e --no-check >> $OUT/other_workloads.jsonl 2>> $OUT/err
 python3 bench.py --scaling strong --config C4 --regions 1250000 --steps 2 --warmup 1 --no-cpu --no-e2e > $OUT/c4_strong_1gpu.json 2>> $OUT/err
-timeout 120 tools/ubench_issue.bin > $OUT/ubench_issue.txt 2>&1
-timeout 120 tools/ubench_ksw.bin > $OUT/ubench_ksw.txt 2>&1
+python3 tools/ubench.py run issue $OUT/ubench_issue.txt || exit 1
+python3 tools/ubench.py run ksw $OUT/ubench_ksw.txt || exit 1
 # what the compiler gave every kernel (registers, spills, scratch, LDS) -- from THESE sources, with their hash in the first line
 python3 - <<'PY' > $OUT/resource_usage.txt 2> $OUT/resource_usage.err
 import os, re, subprocess, sys

@@ -5,7 +5,7 @@
 // VALU -> SGPR -> VALU hop costs (v_readlane, ballot), and the LDS round trip under load.
 // One workgroup of 64*W threads per CU (96 KB of dynamic LDS forces one workgroup per CU), every wave runs the
 // same straight-line block `iters` times and stamps s_memtime around it.
-//   hipcc --offload-arch=gfx950 -O3 -o gpurun_out/ubench_issue tools/ubench_issue.hip && gpurun_out/ubench_issue
+//   tools/ubench.py build, then tools/ubench.py run issue LOG
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdlib.h>

@@ -9,7 +9,7 @@
 //   V6  packed, traceback bits gathered from saturating differences (no compares), packed H
 // The traceback leaves every variant by ordinary vector stores.  (V1, V3 and V5 no longer exist.)
 // Also the issue rate of the few ops the earlier table lacks.
-//   hipcc --offload-arch=gfx950 -O3 -o gpurun_out/ubench_ksw tools/ubench_ksw.hip && gpurun_out/ubench_ksw
+//   tools/ubench.py build, then tools/ubench.py run ksw LOG
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdlib.h>
