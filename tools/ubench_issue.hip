@@ -57,7 +57,7 @@ __global__ void k_bench(Res *out, int iters, int *sink)
 		} else if (KIND == 6) {   // 16 x (v_cmp -> s_and -> v_cndmask -> v_add): ballot-style hop (64 instr)
 			asm volatile(REP8("v_cmp_lt_u32 vcc, %1, %0\n s_and_b64 vcc, vcc, exec\n v_cndmask_b32 %0, %0, %1, vcc\n v_add_u32 %0, %0, 1\n"
 			                  "v_cmp_lt_u32 vcc, %1, %0\n s_and_b64 vcc, vcc, exec\n v_cndmask_b32 %0, %0, %1, vcc\n v_add_u32 %0, %0, 1\n")
-			             : "+v"(v0) : "v"(v1) : "vcc");
+			             : "+v"(v0) : "v"(v1) : "vcc", "scc");
 		} else if (KIND == 7) {   // 16 dependent ds_read_b32 (pointer chase): LDS latency
 			asm volatile(REP8("ds_read_b32 %0, %0\n s_waitcnt lgkmcnt(0)\n ds_read_b32 %0, %0\n s_waitcnt lgkmcnt(0)\n") : "+v"(v0) :: "memory");
 		} else if (KIND == 8) {   // 64 v_pk_add_u16 (8 chains)
