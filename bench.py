@@ -53,10 +53,11 @@ STAGE_MEMBERS = {"k_assemble": ("k_prepack", "k_prepack_fast", "k_slab_expand", 
 
 
 def src_sha16():
-    """Hash of the library's sources: the committed PMC passes carry it, so that a bench line can say whether the counters it
-    quotes were taken from the code it just ran."""
+    """Hash of the library's sources and compiler flags: the committed PMC passes carry it, so that a bench line can say whether
+    the counters it quotes were taken from the code it just ran."""
     import hashlib
-    h = hashlib.sha256()
+    from indelope_amd.build import HIPFLAGS
+    h = hashlib.sha256(" ".join(HIPFLAGS).encode())
     for d in (os.path.join(ROOT, "indelope_amd", "csrc"), os.path.join(ROOT, "include")):
         for f in sorted(os.listdir(d)):
             if f.endswith((".h", ".hip", ".cpp")):

@@ -1,0 +1,44 @@
+"""indelope_amd/build.py: what the compiler is called with, and when (CPU: the compilers are not run)."""
+import os
+import re
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+from indelope_amd import build as B  # noqa: E402
+
+
+@pytest.fixture
+def calls(tmp_path, monkeypatch):
+    """The commands of a build into an empty directory; the "compilers" only leave their output file behind."""
+    seen = []
+
+    def call(cmd, **kw):
+        seen.append(list(cmd))
+        if "-o" in cmd:
+            with open(cmd[cmd.index("-o") + 1], "w") as f:
+                f.write("built %d" % len(seen))
+    monkeypatch.setattr(B.subprocess, "check_call", call)
+    monkeypatch.setattr(B, "LIBDIR", str(tmp_path / "lib"))
+    return seen
+
+
+def test_the_library_is_built_without_packed_fp32(calls):
+    lib, _ = B.build()
+    hip = [c for c in calls if lib in c]
+    assert len(hip) == 1 and hip[0][0] == B.HIPCC
+    assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in " ".join(hip[0])
+    assert "--offload-arch=gfx950" in hip[0] and "-ffp-contract=off" in hip[0]
+
+
+def test_the_evidence_is_of_the_build(monkeypatch):
+    """Counters taken from other flags are of another build; the tools that compile the kernels for a report take the library's flags."""
+    import bench
+    sha = bench.src_sha16()
+    monkeypatch.setattr(B, "HIPFLAGS", B.HIPFLAGS + ["-O2"])
+    assert bench.src_sha16() != sha
+    for f in ("tools/spill_report.py", "tools/profile_round.sh"):
+        text = open(os.path.join(ROOT, f)).read()
+        assert "HIPFLAGS" in text and not re.search(r"offload-arch|ffp-contract|/hipcc", text), f

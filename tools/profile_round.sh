@@ -47,9 +47,10 @@ python3 - <<'PY' > $OUT/resource_usage.txt 2> $OUT/resource_usage.err
 import os, re, subprocess, sys
 sys.path.insert(0, ".")
 import bench
+from indelope_amd.build import HIPCC, HIPFLAGS
 inc, src = "include", "indelope_amd/csrc"
-r = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-I", inc, "-I", src, "-Wno-unused-function",
-                    "-ffp-contract=off", "-Rpass-analysis=kernel-resource-usage", "-o", "/tmp/ihp_ru.so", src + "/indelope_hip.hip"], capture_output=True, text=True)
+r = subprocess.run([HIPCC] + HIPFLAGS + ["-fPIC", "-shared", "-I", inc, "-I", src, "-Wno-unused-function",
+                    "-Rpass-analysis=kernel-resource-usage", "-o", "/tmp/ihp_ru.so", src + "/indelope_hip.hip"], capture_output=True, text=True)
 print("src_sha16 %s  (hipcc -O3 -Rpass-analysis=kernel-resource-usage over indelope_amd/csrc/indelope_hip.hip)" % bench.src_sha16())
 cur = None
 for ln in r.stderr.splitlines():

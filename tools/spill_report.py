@@ -15,6 +15,8 @@ inside `;;#ASMSTART` .. `;;#ASMEND` and that none of those is a spill (the state
 import hashlib, os, re, subprocess, sys, tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+from indelope_amd.build import HIPCC, HIPFLAGS  # noqa: E402
 KERNELS = ["k_ksw_pair", "k_kswILi3E", "k_asm_readsILi8E", "k_asm_combine3ILi5ELb0ELi32E", "k_asm_combine3ILi5ELb0ELi64E", "k_asm_combine3ILi6ELb0ELi32E", "k_asm_combine3ILi4ELb0ELi64ELb1E", "k_tallyILi8E", "k_tally_prep", "k_fallback", "k_prepack_fastILi2ELb0E", "k_prepack_fastILi2ELb1E"]
 
 
@@ -22,14 +24,13 @@ def main():
     out = sys.argv[1] if len(sys.argv) > 1 else None
     src = os.path.join(ROOT, "indelope_amd", "csrc")
     with tempfile.TemporaryDirectory() as td:
-        cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-I", os.path.join(ROOT, "include"), "-I", src,
-               "-Wno-unused-function", "-ffp-contract=off", "-save-temps", "-Rpass-analysis=kernel-resource-usage", "-o", "lib.so", os.path.join(src, "indelope_hip.hip")]
+        cmd = [HIPCC] + HIPFLAGS + ["-fPIC", "-shared", "-I", os.path.join(ROOT, "include"), "-I", src,
+               "-Wno-unused-function", "-save-temps", "-Rpass-analysis=kernel-resource-usage", "-o", "lib.so", os.path.join(src, "indelope_hip.hip")]
         pr = subprocess.run(cmd, cwd=td, capture_output=True, text=True)
         if pr.returncode:
             sys.exit(pr.stderr[-2000:])
         remarks = pr.stderr
         asm = open(os.path.join(td, "indelope_hip-hip-amdgcn-amd-amdhsa-gfx950.s")).read()
-    sys.path.insert(0, ROOT)
     import bench
     lines = ["# scratch (VGPR spill) instructions and SGPR spill moves of the hot kernels by loop depth; sources src_sha16 = %s" % bench.src_sha16(),
              "# depth 0: set-up / epilogue; 1: per work item of the persistent grid; >= 2: inside an item's loops", ""]
