@@ -3,7 +3,8 @@
   lib/libindelope_hip.so  hipcc --offload-arch=gfx950 over csrc/*.hip   (the product)
   lib/libihp_synth.so     g++ over csrc/synth.cpp                        (input generator)
 
-`python -m indelope_amd.build [--force]`.  hipcc cross-compiles without a GPU.
+`python -m indelope_amd.build [--force]`: what is older than its sources or, for the product, than the flags in this file; all of it
+with --force.  hipcc cross-compiles without a GPU.
 """
 import os
 import subprocess
@@ -42,7 +43,7 @@ def build(force=False, verbose=False):
     # product
     lib = os.path.join(LIBDIR, "libindelope_hip.so")
     hips = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
-    if hips and (force or _stale(lib, hips + hdrs)):
+    if hips and (force or _stale(lib, hips + hdrs + [os.path.abspath(__file__)])):
         cmd = [HIPCC] + HIPFLAGS + ["-fPIC", "-shared", "-I", INC, "-I", CSRC, "-Wall", "-Wno-unused-function",
                                     "-o", lib] + hips + ["-ldl"]      # dlopen: librccl.so.1 is opened by the first ihp_dist_* call, not linked
         if os.environ.get("IHP_SAVE_TEMPS"):

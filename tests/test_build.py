@@ -42,3 +42,25 @@ def test_the_evidence_is_of_the_build(monkeypatch):
     for f in ("tools/spill_report.py", "tools/profile_round.sh"):
         text = open(os.path.join(ROOT, f)).read()
         assert "HIPFLAGS" in text and not re.search(r"offload-arch|ffp-contract|/hipcc", text), f
+
+
+def test_a_change_of_the_flags_builds_again(calls, monkeypatch):
+    lib, _ = B.build()
+    n = len(calls)
+    B.build()
+    assert len(calls) == n                                       # nothing to do
+    t = os.path.getmtime(B.__file__) - 10
+    os.utime(lib, (t, t))
+    mtime = os.path.getmtime
+    monkeypatch.setattr(B.os.path, "getmtime", lambda p: t - 10 if p.endswith((".hip", ".h")) else mtime(p))
+    B.build()
+    assert len(calls) == n + 1 and lib in calls[-1]
+
+
+def test_the_build_entry_compiles_what_is_there_too(calls):
+    import __graft_entry__
+    __graft_entry__.build()
+    first = [c for c in calls if c[0] in ("g++", B.HIPCC)]
+    del calls[:]
+    __graft_entry__.build()
+    assert len(first) == 2 and [c for c in calls if c[0] in ("g++", B.HIPCC)] == first
