@@ -7,15 +7,17 @@
 #   C3 / C5 kernel stats and bench lines, C2 variants (--quals, --dup-frac 0.1, --sub-batches 1), a C4 strong-scaling
 #   run on this one GPU (1.25 M regions in 8 resident chunks), the issue-rate microbenchmark.
 cd "$(dirname "$0")/.." || exit 1
+set -eo pipefail                             # a step that failed, faulted or ran into its limit ends the script: nothing more is started on the GPU
+T="timeout -k 10 240"
 export TMPDIR=/tmp
 python3 tools/ubench.py check || exit 1      # (built on the build host: tools/ubench.py build)
 OUT=gpurun_out/prof
 rm -rf $OUT; mkdir -p $OUT
 ARGS="--steps 5 --warmup 2 --no-cpu --no-e2e --no-check --no-other"
-stats() { name=$1; shift; rocprofv3 --kernel-trace --stats --output-format csv -d $OUT/$name -- python3 bench.py "$@" > $OUT/$name.log 2>&1; f=$(find $OUT/$name -name "*kernel_stats.csv" | head -1); [ -n "$f" ] && cp $f $OUT/${name}_kernel_stats.csv; }
+stats() { name=$1; shift; $T rocprofv3 --kernel-trace --stats --output-format csv -d $OUT/$name -- python3 bench.py "$@" > $OUT/$name.log 2>&1; f=$(find $OUT/$name -name "*kernel_stats.csv" | head -1); cp $f $OUT/${name}_kernel_stats.csv; echo "$name done"; }
 stats c2 $ARGS
-rocprofv3 --pmc FETCH_SIZE --output-format csv -d $OUT/fetch -- python3 bench.py $ARGS > $OUT/fetch.log 2>&1
-rocprofv3 --pmc WRITE_SIZE --output-format csv -d $OUT/write -- python3 bench.py $ARGS > $OUT/write.log 2>&1
+$T rocprofv3 --pmc FETCH_SIZE --output-format csv -d $OUT/fetch -- python3 bench.py $ARGS > $OUT/fetch.log 2>&1
+$T rocprofv3 --pmc WRITE_SIZE --output-format csv -d $OUT/write -- python3 bench.py $ARGS > $OUT/write.log 2>&1
 python3 tools/pmc_sum.py $OUT/fetch $OUT/write --last 10 --json $OUT/pmc_raw.json > $OUT/pmc_raw.txt 2>&1
 bash tools/pmc_mix.sh > /dev/null 2>&1
 cp gpurun_out/pmc_mix/mix.json $OUT/c2_pmc_mix.json
@@ -23,23 +25,23 @@ STEADY="--no-cpu --no-e2e --no-check --no-other --regions 100000 --steps 3 --war
 stats steady100k $STEADY
 PMC_LAST=3 bash tools/pmc_mix.sh --regions 100000 --in-flight 1 --sub-batches 1 > /dev/null 2>&1
 cp gpurun_out/pmc_mix/mix.json $OUT/steady100k_pmc_mix.json
-python3 bench.py $STEADY > $OUT/steady100k_bench.json 2>> $OUT/err
+$T python3 bench.py $STEADY > $OUT/steady100k_bench.json 2>> $OUT/err
 stats c3 --config C3 --steps 3 --warmup 1 --no-cpu --no-e2e --no-check
 stats c5 --config C5 --steps 5 --warmup 2 --no-cpu --no-e2e --no-check
 # round 6: the regions of 257-600 reads (wide combine build): the byte-based k_assemble passes must stay empty
 stats deep --config deep --regions 10000 --steps 3 --warmup 2 --in-flight 1 --sub-batches 2 --no-cpu --no-e2e --no-check
-python3 bench.py --config deep --regions 10000 --steps 3 --warmup 2 --in-flight 1 --sub-batches 2 --no-cpu --no-e2e > $OUT/deep_bench.json 2>> $OUT/err
+$T python3 bench.py --config deep --regions 10000 --steps 3 --warmup 2 --in-flight 1 --sub-batches 2 --no-cpu --no-e2e > $OUT/deep_bench.json 2>> $OUT/err
 python3 tools/ubench.py run wany $OUT/ubench_wany.txt || exit 1
 : > $OUT/other_workloads.jsonl
-python3 bench.py --config C3 --steps 3 --warmup 1 --no-cpu --no-e2e >> $OUT/other_workloads.jsonl 2>> $OUT/err
-python3 bench.py --config C5 --no-cpu --no-e2e >> $OUT/other_workloads.jsonl 2>> $OUT/err
-python3 bench.py --no-cpu --no-e2e --no-check --no-other --quals >> $OUT/other_workloads.jsonl 2>> $OUT/err
-python3 bench.py --no-cpu --no-e2e --no-check --no-other --dup-frac 0.1 >> $OUT/other_workloads.jsonl 2>> $OUT/err
-python3 bench.py --no-cpu --no-e2e --no-check --no-other --in-flight 1 --sub-batches 1 >> $OUT/other_workloads.jsonl 2>> $OUT/err
-python3 bench.py --no-cpu --no-e2e --no-check --no-other --in-flight 1 --lockstep >> $OUT/other_workloads.jsonl 2>> $OUT/err
-python3 bench.py --knob asm_v1=1 --no-cpu --no-e2e --no-check --no-other >> $OUT/other_workloads.jsonl 2>> $OUT/err
-python3 bench.py --config C3 --knob no_rich=1 --steps 3 --warmup 1 --no-cpu --no-e2e --no-check >> $OUT/other_workloads.jsonl 2>> $OUT/err
-python3 bench.py --scaling strong --config C4 --regions 1250000 --steps 2 --warmup 1 --no-cpu --no-e2e > $OUT/c4_strong_1gpu.json 2>> $OUT/err
+$T python3 bench.py --config C3 --steps 3 --warmup 1 --no-cpu --no-e2e >> $OUT/other_workloads.jsonl 2>> $OUT/err
+$T python3 bench.py --config C5 --no-cpu --no-e2e >> $OUT/other_workloads.jsonl 2>> $OUT/err
+$T python3 bench.py --no-cpu --no-e2e --no-check --no-other --quals >> $OUT/other_workloads.jsonl 2>> $OUT/err
+$T python3 bench.py --no-cpu --no-e2e --no-check --no-other --dup-frac 0.1 >> $OUT/other_workloads.jsonl 2>> $OUT/err
+$T python3 bench.py --no-cpu --no-e2e --no-check --no-other --in-flight 1 --sub-batches 1 >> $OUT/other_workloads.jsonl 2>> $OUT/err
+$T python3 bench.py --no-cpu --no-e2e --no-check --no-other --in-flight 1 --lockstep >> $OUT/other_workloads.jsonl 2>> $OUT/err
+$T python3 bench.py --knob asm_v1=1 --no-cpu --no-e2e --no-check --no-other >> $OUT/other_workloads.jsonl 2>> $OUT/err
+$T python3 bench.py --config C3 --knob no_rich=1 --steps 3 --warmup 1 --no-cpu --no-e2e --no-check >> $OUT/other_workloads.jsonl 2>> $OUT/err
+$T python3 bench.py --scaling strong --config C4 --regions 1250000 --steps 2 --warmup 1 --no-cpu --no-e2e > $OUT/c4_strong_1gpu.json 2>> $OUT/err
 python3 tools/ubench.py run issue $OUT/ubench_issue.txt || exit 1
 python3 tools/ubench.py run ksw $OUT/ubench_ksw.txt || exit 1
 # what the compiler gave every kernel (registers, spills, scratch, LDS) -- from THESE sources, with their hash in the first line
@@ -65,9 +67,9 @@ for ln in r.stderr.splitlines():
     elif cur:
         print("    " + t)
 PY
-python3 bench.py > $OUT/bench.json 2> $OUT/bench.err
-python3 bench.py --no-cpu --no-e2e --no-other --no-check --profile --in-flight 1 --sub-batches 1 > $OUT/c2_phase_cycles.json 2>> $OUT/err
-python3 bench.py --config C5 --no-cpu --no-e2e --no-other --no-check --profile --in-flight 1 --sub-batches 1 > $OUT/c5_phase_cycles.json 2>> $OUT/err
+$T python3 bench.py > $OUT/bench.json 2> $OUT/bench.err
+$T python3 bench.py --no-cpu --no-e2e --no-other --no-check --profile --in-flight 1 --sub-batches 1 > $OUT/c2_phase_cycles.json 2>> $OUT/err
+$T python3 bench.py --config C5 --no-cpu --no-e2e --no-other --no-check --profile --in-flight 1 --sub-batches 1 > $OUT/c5_phase_cycles.json 2>> $OUT/err
 python3 - <<'PY'
 import json, sys
 sys.path.insert(0, ".")
@@ -95,8 +97,8 @@ for k, v in raw.items():
 json.dump(out, open("gpurun_out/prof/c2_pmc.json", "w"), indent=1)
 PY
 # round 5: the PCIe-inclusive leg on the compact slab (host buffers in -> host buffers out), the host's share of an upload
-python3 bench.py --no-cpu --no-other --no-check > $OUT/e2e_bench.json 2>> $OUT/err
-python3 tools/e2e_host_time.py > $OUT/e2e_host_time.txt 2>&1
+$T python3 bench.py --no-cpu --no-other --no-check > $OUT/e2e_bench.json 2>> $OUT/err
+$T python3 tools/e2e_host_time.py > $OUT/e2e_host_time.txt 2>&1
 # round 4: the alignment fallback under load (C2 with 10 % duplications), k_prepack vs k_prepack_fast, the pair sweep's instruction mix
 bash tools/r4_fb.sh > $OUT/dup10_summary.txt 2>&1
 cp gpurun_out/fb/kernel_stats.csv $OUT/dup10_kernel_stats.csv; cp gpurun_out/fb/mix.json $OUT/dup10_pmc_mix.json
@@ -131,5 +133,5 @@ PY
 # the raw rocprofv3 output directories are large (gpurun merges at most 64 MiB back): keep the summaries only
 rm -rf $OUT/c2 $OUT/steady100k $OUT/c3 $OUT/c5 $OUT/fetch $OUT/write gpurun_out/pmc_mix/g1 gpurun_out/pmc_mix/g2 gpurun_out/pmc_mix/g3
 du -sh gpurun_out
-cat $OUT/bench.json | head -c 1500
+head -c 1500 $OUT/bench.json
 head -14 $OUT/c2_kernel_stats.csv | cut -c1-150
