@@ -498,7 +498,8 @@ def break_even(api, K=27, sizes=(1, 2, 4, 8, 16, 32, 64, 128, 256, 512, 1024), r
     key = "cpu_%dthreads_us" % usable
     be1 = next((r["regions"] for r in rows if r["gpu_us"] < r["cpu_1thread_us"]), None)
     bem = next((r["regions"] for r in rows if r["gpu_us"] < r[key]), None)
-    return {"workload": "n C2-shaped regions (64 x 150 bp) through ihp_run_regions (pageable arrays in, results out) vs the C oracle with the compiled reference ksw2",
+    return {"workload": "n C2-shaped regions (64 x 150 bp) through ihp_run_regions (pageable arrays in, results out) vs the C oracle (ksw2 = %s)"
+                        % ("reference ksw2_extz2_sse.c compiled (oracle/_ref)" if used_ref else "scalar restatement (oracle/_ref absent)"),
             "rows": rows, "gpu_faster_than_one_cpu_thread_from": be1, "gpu_faster_than_%d_cpu_threads_from" % usable: bem, "cpu_threads": usable}
 
 
