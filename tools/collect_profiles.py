@@ -3,7 +3,7 @@
 Files that carry the hash of the library sources they were taken from (`src_sha16` / `_src_sha16`: the PMC passes, the bench
 lines, the compiler's resource usage) are REFUSED when that hash is not the one of the sources in the tree: evidence of
 another build is not this round's evidence.
-usage: tools/collect_profiles.py r04"""
+usage: tools/collect_profiles.py [current]"""
 import json
 import os
 import re
@@ -13,7 +13,7 @@ import sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 src = os.path.join(ROOT, "gpurun_out", "prof")
 dst = os.path.join(ROOT, "profiles")
-pre = sys.argv[1] if len(sys.argv) > 1 else "r06"
+pre = sys.argv[1] if len(sys.argv) > 1 else "current"
 sys.path.insert(0, ROOT)
 import bench  # noqa: E402
 
