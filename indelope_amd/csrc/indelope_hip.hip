@@ -4,7 +4,7 @@
 // sizes the per-workgroup scratch, launches assemble -> ksw2 -> tally -> summary
 // on one stream, and repacks the slot-indexed device outputs into the flat
 // `ihp_batch_out`.  The only arithmetic done on the host is genotype()
-// (genotyper.nim:36-47: three fp64 logs per event).  There is no CPU fallback.
+// (genotyper.nim:36-47: seven fp64 logs per event).  There is no CPU fallback.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdio.h>
