@@ -53,17 +53,26 @@ STAGE_MEMBERS = {"k_assemble": ("k_prepack", "k_prepack_fast", "k_slab_expand", 
 
 
 def src_sha16():
-    """Hash of the library's sources and compiler flags: the committed PMC passes carry it, so that a bench line can say whether
-    the counters it quotes were taken from the code it just ran."""
+    """Hash of the library's code and compiler flags: the committed PMC passes carry it, so that a bench line can say whether the
+    counters it quotes were taken from the code it just ran.  Comments and white space do not count: they change no kernel."""
     import hashlib
     from indelope_amd.build import HIPFLAGS
     h = hashlib.sha256(" ".join(HIPFLAGS).encode())
     for d in (os.path.join(ROOT, "indelope_amd", "csrc"), os.path.join(ROOT, "include")):
         for f in sorted(os.listdir(d)):
             if f.endswith((".h", ".hip", ".cpp")):
-                h.update(f.encode())
-                h.update(open(os.path.join(d, f), "rb").read())
+                with open(os.path.join(d, f), encoding="latin-1") as fh:
+                    h.update((f + "\n" + _code(fh.read())).encode("latin-1"))
     return h.hexdigest()[:16]
+
+
+def _code(text):
+    """C++ source without its comments; a run of white space is one space, or one line end where it holds one.  Strings and
+    characters stay as they are (a quote behind a digit separates digits)."""
+    import re
+    keep = r'"(?:\\.|[^"\\\n])*"|(?<![0-9A-Fa-f])\'(?:\\.|[^\'\\\n])+\''
+    drop = r"(?:\s|//[^\n]*|/\*.*?\*/)+"
+    return re.sub("(%s)|%s" % (keep, drop), lambda m: m.group(1) or ("\n" if "\n" in m.group(0) else " "), text, flags=re.S).strip()
 
 
 class _DevArray:

@@ -1,6 +1,7 @@
 """indelope_amd/build.py: what the compiler is called with, and when (CPU: the compilers are not run)."""
 import os
 import re
+import shutil
 import sys
 
 import pytest
@@ -64,3 +65,42 @@ def test_the_build_entry_compiles_what_is_there_too(calls):
     del calls[:]
     __graft_entry__.build()
     assert len(first) == 2 and [c for c in calls if c[0] in ("g++", B.HIPCC)] == first
+
+
+@pytest.fixture
+def sources(tmp_path, monkeypatch):
+    """bench.py on a copy of the library's sources."""
+    import bench
+    for d in (("indelope_amd", "csrc"), ("include",)):
+        shutil.copytree(os.path.join(ROOT, *d), str(tmp_path.joinpath(*d)))
+    monkeypatch.setattr(bench, "ROOT", str(tmp_path))
+    return bench, tmp_path / "indelope_amd" / "csrc"
+
+
+def test_a_comment_makes_no_other_build(sources):
+    """A changed comment left the committed counters marked as another build's."""
+    bench, csrc = sources
+    sha = bench.src_sha16()
+    f = csrc / "kernels.h"
+    text = f.read_text()
+    f.write_text("// a remark\n/* and one\n   of 2 lines */\n" + text.replace(";\n", ";   // \"quoted\" and it's fine\n\n", 50))
+    assert bench.src_sha16() == sha
+    f.write_text(text + "\n__device__ int one_more;\n")
+    assert bench.src_sha16() != sha
+
+
+@pytest.mark.parametrize("a,b", [
+    ('x = "a // b";', 'x = "a // c";'), ('x = "a  b";', 'x = "a b";'), ("x = '\"'; y = 1; // '", "x = '\"'; y = 2; // '"),
+    ("x = 0x49'4c; y = 1;", "x = 0x49'4c; y = 2;"), ('x = "\\"/*"; y = 1; /**/', 'x = "\\"/*"; y = 2; /**/'),
+    ("#define A 1\nB", "#define A 1 B"), ("a /* c */ b", "ab"), ("x = '/'; y = 1;", "x = '/'; y = 2;")])
+def test_a_change_of_code_makes_another_build(a, b):
+    import bench
+    assert bench._code(a) != bench._code(b)
+
+
+@pytest.mark.parametrize("a,b", [
+    ("x = 1; // one", "x = 1;"), ("x = 1;\n// one\ny = 2;", "x = 1;\n\ty = 2;  /* two */\n"), ("x = 'a'; // 'b", "x = 'a';"),
+    ('x = "a"; /* " */ y = 1;', 'x = "a"; y = 1;')])
+def test_what_is_no_code(a, b):
+    import bench
+    assert bench._code(a) == bench._code(b)
