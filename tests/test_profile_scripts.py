@@ -47,3 +47,64 @@ def test_every_step_on_the_gpu_has_a_limit(script):
     assert 'T="timeout -k 10 ' in code
     steps = [m.start() for m in re.finditer(r"(?<!-- )(?:rocprofv3 --\w|python3 bench\.py)", code)]
     assert steps and all(code[:i].endswith("$T ") for i in steps)
+
+
+# every script that starts something on the GPU; the stand-ins count those steps and fail the one that is asked for
+ALL = sorted(f[:-3] for f in os.listdir(os.path.join(ROOT, "tools")) if f.endswith(".sh"))
+ARGS = {"r5_occ": ["a=1", "b=2"], "r6_stats": ["name"]}                # what the others take has a default
+STAND_IN = r"""#!/bin/bash
+me=$(basename "$0"); d=.; j=; prev=
+for a in "$@"; do [ "$prev" = -d ] && d=$a; [ "$prev" = --json ] && j=$a; prev=$a; done
+case "$me $*" in
+  "rocprofv3 "*|*bench.py*|*_stress.py*|*stress_parity.py*|*"-m pytest"*|*e2e_host_time.py*|*"ubench.py run"*) ;;
+  *) [ -n "$j" ] && echo "{}" > "$j"; [ "$1" = -c ] && cat > /dev/null; echo "k_ksw_pair avg 1 us 1 %"; exit 0;;
+esac
+echo "$me $*" >> "$CALLS"
+[ "$(wc -l < "$CALLS")" = "$FAIL_AT" ] && exit "$STATUS"
+if [ "$me" = rocprofv3 ]; then mkdir -p "$d"; echo k_ksw_pair,k_prepack > "$d/1_kernel_stats.csv"; cp "$d/1_kernel_stats.csv" "$d/1_kernel_trace.csv"; fi
+echo '{"metric k_ksw_pair'
+"""
+
+
+def _steps(tmp_path, script, fail_at, status):
+    """(exit status, GPU steps started) of the script when its `fail_at`-th GPU step ends with `status`."""
+    (tmp_path / "tools").mkdir()
+    for s in ALL:
+        shutil.copy(os.path.join(ROOT, "tools", s + ".sh"), tmp_path / "tools")
+    lib, bin_, log = tmp_path / "indelope_amd" / "lib", tmp_path / "bin", tmp_path / "calls"
+    lib.mkdir(parents=True)
+    for so in ("libindelope_hip", "ab_one", "ab_two"):
+        (lib / (so + ".so")).write_text(so)
+    bin_.mkdir()
+    log.write_text("")
+    for name in ("rocprofv3", "python3", "python"):
+        (bin_ / name).write_text(STAND_IN)
+        (bin_ / name).chmod(0o755)
+    env = dict(os.environ, PATH="%s:%s" % (bin_, os.environ["PATH"]), CALLS=str(log), FAIL_AT=str(fail_at), STATUS=str(status))
+    r = subprocess.run(["bash", str(tmp_path / "tools" / (script + ".sh"))] + ARGS.get(script, []), env=env, stdin=subprocess.DEVNULL, capture_output=True,
+                       timeout=100)
+    assert (lib / "libindelope_hip.so").read_text() == "libindelope_hip"
+    return r.returncode, log.read_text().splitlines()
+
+
+@pytest.mark.parametrize("script", ALL)
+def test_no_script_goes_on_after_a_failed_step(tmp_path, script):
+    rc, steps = _steps(tmp_path, script, 0, 0)
+    n = len(steps)
+    assert n and rc == 0
+    for i in sorted({1, 2, 3, n} & set(range(1, n + 1))):
+        (tmp_path / str(i)).mkdir()
+        rc, steps = _steps(tmp_path / str(i), script, i, 139)
+        assert rc != 0 and len(steps) == i, (i, rc, steps)
+
+
+@pytest.mark.parametrize("script", ALL)
+def test_every_step_of_every_script_has_a_limit_that_kills(script):
+    """`timeout` without -k leaves a process that ignores the first signal; rocprofv3 does after some errors."""
+    with open(os.path.join(ROOT, "tools", script + ".sh")) as f:
+        code = "".join(ln for ln in f if not ln.lstrip().startswith(("#", '"')))
+    assert not re.search(r"timeout (?!-k 10 )", code)
+    steps = [m.start() for m in re.finditer(r"(?<!-- )(?:rocprofv3 --\w|python3? (?:bench\.py|-m pytest|tools/\w*stress\w*\.py))", code)]
+    for i in steps:
+        assert re.search(r"(?:\$T |timeout -k 10 \d+ |^run \w+ )$", code[:i], flags=re.M), code[i:i + 60]
+    assert steps

@@ -1,7 +1,8 @@
 cd "$(dirname "$0")/.." || exit 1
+set -eo pipefail                             # a step that failed, faulted or ran into its limit ends the script: nothing more is started on the GPU
 mkdir -p gpurun_out/stress
 S=${1:-201}
-run() { name=$1; shift; timeout 2400 "$@" > gpurun_out/stress/$name.txt 2>&1; echo "== $name rc=$? : $(tail -1 gpurun_out/stress/$name.txt | cut -c1-200)"; grep -c DIFF gpurun_out/stress/$name.txt; }
+run() { name=$1; rc=0; shift; timeout -k 10 2400 "$@" > gpurun_out/stress/$name.txt 2>&1 || rc=$?; echo "== $name rc=$rc : $(tail -1 gpurun_out/stress/$name.txt | cut -c1-200)"; grep -c DIFF gpurun_out/stress/$name.txt || true; return $rc; }
 run pair_a python tools/ksw_pair_stress.py $S 700
 run pair_b python tools/ksw_pair_stress.py $((S+1)) 700
 run ksw python tools/ksw_stress.py $S 1000

@@ -2,9 +2,10 @@
 # Round-6 randomised runs on the final sources (one gpurun call): round 5's harnesses + regions of 200-700 reads (the wide combine
 # build, the byte-based passes above 640 reads and 64 contigs) + the compact fetch.   tools/r6_stress.sh [seed] [scale]
 cd "$(dirname "$0")/.." || exit 1
+set -eo pipefail                             # a step that failed, faulted or ran into its limit ends the script: nothing more is started on the GPU
 mkdir -p gpurun_out/stress
 S=${1:-61}; X=${2:-1}
-run() { name=$1; shift; timeout 2400 "$@" > gpurun_out/stress/$name.txt 2>&1; echo "== $name rc=$? : $(tail -1 gpurun_out/stress/$name.txt | cut -c1-200)"; grep -c DIFF gpurun_out/stress/$name.txt; }
+run() { name=$1; rc=0; shift; timeout -k 10 2400 "$@" > gpurun_out/stress/$name.txt 2>&1 || rc=$?; echo "== $name rc=$rc : $(tail -1 gpurun_out/stress/$name.txt | cut -c1-200)"; grep -c DIFF gpurun_out/stress/$name.txt || true; return $rc; }
 run pair_a python tools/ksw_pair_stress.py $S $((150*X))
 run ksw python tools/ksw_stress.py $S $((250*X))
 run regions_params python tools/stress_parity.py $((300*X)) $S params

@@ -1,9 +1,11 @@
 #!/bin/bash
 # one steady-state step (100 000 regions, one chain) kernel by kernel: start and end of every launch relative to the step's first
 cd "$(dirname "$0")/.." || exit 1
+set -eo pipefail                             # a step that failed, faulted or ran into its limit ends the script: nothing more is started on the GPU
+T="timeout -k 10 240"
 export TMPDIR=/tmp
 OUT=gpurun_out/trace; rm -rf $OUT; mkdir -p $OUT
-rocprofv3 --kernel-trace --output-format csv -d $OUT/run -- python3 bench.py --no-cpu --no-e2e --no-check --no-other --regions ${1:-100000} --steps 3 --warmup 1 --in-flight 1 --sub-batches 1 > $OUT/log 2>&1
+$T rocprofv3 --kernel-trace --output-format csv -d $OUT/run -- python3 bench.py --no-cpu --no-e2e --no-check --no-other --regions ${1:-100000} --steps 3 --warmup 1 --in-flight 1 --sub-batches 1 > $OUT/log 2>&1
 f=$(find $OUT/run -name "*kernel_trace.csv" | head -1)
 python3 - "$f" <<'PY'
 import csv, sys
