@@ -4,6 +4,7 @@ import os
 import re
 import shutil
 import subprocess
+import sys
 
 import pytest
 
@@ -108,3 +109,23 @@ def test_every_step_of_every_script_has_a_limit_that_kills(script):
     for i in steps:
         assert re.search(r"(?:\$T |timeout -k 10 \d+ |^run \w+ )$", code[:i], flags=re.M), code[i:i + 60]
     assert steps
+
+
+@pytest.mark.parametrize("script,shown", [("r6_stats", "5.25 {}"), ("r5_kstats", "5.25 7.5")])
+def test_the_bench_line_is_found_before_the_profilers_last_words(tmp_path, script, shown):
+    (tmp_path / "tools").mkdir()
+    shutil.copy(os.path.join(ROOT, "tools", script + ".sh"), tmp_path / "tools")
+    bin_ = tmp_path / "bin"
+    bin_.mkdir()
+    (bin_ / "rocprofv3").write_text("""#!/bin/bash
+while [ "$1" != -d ]; do shift; done
+mkdir -p "$2"; echo Name > "$2/1_kernel_stats.csv"
+echo '{"metric": "m", "value": 5.25, "ms_per_step": 7.5, "kernel_ms": {}}'
+echo "the profiler's last words"
+""")
+    (bin_ / "python3").write_text('#!/bin/bash\n[ "$1" != -c ] || exec %s "$@"\n' % sys.executable)
+    for f in bin_.iterdir():
+        f.chmod(0o755)
+    r = subprocess.run(["bash", str(tmp_path / "tools" / (script + ".sh")), "steady"], stdin=subprocess.DEVNULL, capture_output=True, text=True, timeout=100,
+                       env=dict(os.environ, PATH="%s:%s" % (bin_, os.environ["PATH"])))
+    assert r.returncode == 0 and shown in r.stdout, (r.stdout, r.stderr)

@@ -7,7 +7,7 @@ T="timeout -k 10 240"
 export TMPDIR=/tmp
 OUT=gpurun_out/ks; rm -rf $OUT; mkdir -p $OUT
 run() { name=$1; shift; $T rocprofv3 --kernel-trace --stats --output-format csv -d $OUT/$name -- python3 bench.py "$@" $KNOBS > $OUT/$name.log 2>&1
-  f=$(find $OUT/$name -name "*kernel_stats.csv" | head -1); echo "== $name: $(tail -1 $OUT/$name.log | python3 -c 'import json,sys; d=json.loads(sys.stdin.read()); print(d["value"], d["ms_per_step"])' 2>/dev/null)"
+  f=$(find $OUT/$name -name "*kernel_stats.csv" | head -1); echo "== $name: $(grep '^{"metric' $OUT/$name.log | python3 -c 'import json,sys; d=json.loads(sys.stdin.read()); print(d["value"], d["ms_per_step"])' 2>/dev/null)"
   [ -n "$f" ] && python3 - "$f" <<'PY'
 import csv, sys
 rows = [r for r in csv.DictReader(open(sys.argv[1])) if "ihp::" in r["Name"]]

@@ -16,4 +16,4 @@ for r in rows[:14]:
     print("%-62s calls %5s avg %10.1f us  %5.1f %%" % (r["Name"][:62], r["Calls"], float(r["AverageNs"]) / 1e3, float(r["Percentage"])))
 PY
 rm -rf $OUT/run_$NAME
-tail -1 $OUT/$NAME.log | python3 -c "import json,sys; d=json.loads(sys.stdin.read()); print(d['value'], d['kernel_ms'])"
+grep '^{"metric' $OUT/$NAME.log | python3 -c "import json,sys; d=json.loads(sys.stdin.read()); print(d['value'], d['kernel_ms'])"
